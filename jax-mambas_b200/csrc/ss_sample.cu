@@ -306,7 +306,8 @@ __device__ __forceinline__ void push(SampleShared& sh, unsigned long long key) {
 
 // After the CTAs' lists are complete: their joint length in every thread (more
 // than kSortCap: not joined), and rank 0's list is all of them. Ends with a
-// barrier after the last access to another CTA's memory.
+// barrier after the last access to another CTA's memory; a row's only CTA has none after
+// its read of sh.count, so who sets that anew waits for its threads first.
 __device__ int join_lists(SampleShared& sh, int rank, int ctas) {
   sync_row(ctas);
   if (ctas == 1) return static_cast<int>(sh.count);
@@ -768,7 +769,9 @@ __global__ void __launch_bounds__(kSampleThreads, kCtasPerSm)
       }
       return;
     }
-    if (threadIdx.x == 0) sh.count = 0;  // too many equal logits: the general way
+    // too many equal logits: the general way
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;  // counted in again after another barrier
   }
 
   // ---- cutoff of top-k and top-p

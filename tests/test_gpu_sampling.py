@@ -270,3 +270,25 @@ def test_parameters_that_are_not_numbers(name):
             sample_tokens(z, u, **{name: bad})
     one = np.float32(1.0) if name != "top_k" else np.int32(1)
     assert sample_tokens(z, u, **{name: one}).shape == (2,)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(200, 5000), (600, 5000), (300, 9001)])
+@pytest.mark.parametrize("kw", [{"top_k": 2}, {"top_k": 50}, {"top_k": 300},
+                                {"top_k": 50, "top_p": 0.5}, {"top_k": 300, "top_p": 0.5},
+                                {"top_k": 500, "top_p": 0.9}],
+                         ids=lambda k: "-".join(f"{a}{b}" for a, b in k.items()))
+def test_more_candidates_than_a_list_holds(rows, vocab, kw, dtype):
+    """Rows of one CTA each whose bound leaves more than 2048 candidates: all equal, all
+    equal but a few above, and equal where a mask leaves them. The draw then goes from the
+    list to the general way, in every thread of the CTA."""
+    z = torch.zeros(rows, vocab, device="cuda", dtype=dtype)
+    z[1::3, 7], z[1::3, vocab - 3] = 1.0, 2.0
+    z[2::3, ::2] = -float("inf")
+    u, want = np.zeros(rows), np.zeros(rows, int)
+    for kind in range(3):
+        us, ws = _middles(z[kind].double().cpu().numpy(), 31, **kw)
+        at = np.arange(kind, rows, 3)
+        u[at], want[at] = us[at % us.size], ws[at % ws.size]
+    for _ in range(4):
+        np.testing.assert_array_equal(_run(z, u, **kw), want)
