@@ -1006,10 +1006,11 @@ static cudaError_t sample_go(const SampleParams& p, cudaStream_t stream) {
   // run under the others' barriers), and more while there are fewer CTAs than SMs and
   // slices of at least 2048 remain
   auto slice = [&](int c) { return ((p.vocab + c - 1) / c + 7) / 8 * 8; };
-  auto need = [&](int c) {
-    const size_t units = (slice(c) + kUnit - 1) / kUnit;
+  auto bytes_of = [](size_t elems) {
+    const size_t units = (elems + kUnit - 1) / kUnit;
     return sizeof(SampleShared) + (units + 1) / 2 * 16 + units * kUnit * sizeof(T);
   };
+  auto need = [&](int c) { return bytes_of(slice(c)); };
   int ctas = 1;
   constexpr size_t kThirdOfSm = 75 * 1024;
   while (ctas < 8 && need(ctas) > kThirdOfSm) ctas *= 2;
@@ -1032,8 +1033,11 @@ static cudaError_t sample_go(const SampleParams& p, cudaStream_t stream) {
   };
   const int per_sm = bytes <= kThirdOfSm && rounds(3) < rounds(2) ? 3 : 2;
   auto fn = per_sm == 3 ? ss_sample_kernel<T, 3> : ss_sample_kernel<T, 2>;
+  // The limit is the function's, shared by all host threads: the same in every call, the
+  // most that any call of this form takes.
+  const size_t most = per_sm == 3 ? kThirdOfSm : bytes_of(kSampleMaxSlice);
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(bytes));
+                                             static_cast<int>(most));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * ctas, 1, 1);

@@ -292,3 +292,40 @@ def test_more_candidates_than_a_list_holds(rows, vocab, kw, dtype):
         u[at], want[at] = us[at % us.size], ws[at % ws.size]
     for _ in range(4):
         np.testing.assert_array_equal(_run(z, u, **kw), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_from_several_host_threads(dtype):
+    """Through the C interface, whose calls run at the same time in several host threads:
+    rows that need most of an SM's shared memory, and rows that need little."""
+    import threading
+
+    from mamba import _native
+
+    lib = _native.load()
+    code = {F32: 0, BF16: 1}[dtype]
+    failed = []
+
+    def calls(vocab):
+        z = torch.zeros(4, vocab, device="cuda", dtype=dtype)
+        z[:, 5] = 9.0
+        u = torch.rand(4, device="cuda")
+        t = torch.empty(4, dtype=torch.int64, device="cuda")
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        for _ in range(3000):
+            if lib.mamba_ss_sample_tokens(s.cuda_stream, code, 4, vocab, z.data_ptr(), vocab,
+                                          u.data_ptr(), None, None, None, None, 0.0, 0, 1.0, 0.0,
+                                          t.data_ptr()):
+                failed.append((vocab, lib.mamba_ss_last_error()))
+                break
+        s.synchronize()
+        if not (t == 5).all():
+            failed.append((vocab, t.tolist()))
+
+    threads = [threading.Thread(target=calls, args=(v,)) for v in (360448, 64, 9000, 1000)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed
