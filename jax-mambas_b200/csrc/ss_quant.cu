@@ -140,9 +140,9 @@ __global__ void __launch_bounds__(256) ss_quant_cm_kernel(const QuantParams p) {
   __syncthreads();
   if (threadIdx.x < kTileL) {  // one thread per position joins the warps' maxima
     const int l = threadIdx.x;
-    float a = wmax[0][l];
+    float a = 0.f;  // of a position of nothing but NaN, whose maxima are NaN
 #pragma unroll
-    for (int w = 1; w < 8; ++w) a = fmaxf(a, wmax[w][l]);
+    for (int w = 0; w < 8; ++w) a = fmaxf(a, wmax[w][l]);
     const int byte = scale_byte(a);
     inverse[l] = scale_inverse(byte);
     if (l0 + l < p.length)
