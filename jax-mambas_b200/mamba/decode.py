@@ -25,12 +25,12 @@ class _Layer:
 
     def __init__(self, block, dtype):
         quant = lambda w: quantize_fp8(w.detach().to(dtype))  # noqa: E731
-        f32 = lambda w: w.detach().float().contiguous()  # noqa: E731
+        f32 = lambda w: w.detach().to(torch.float32, copy=True).contiguous()  # noqa: E731
         self.norm = f32(block.norm.weight)
         self.w_main, self.w_skip = quant(block.w_main), quant(block.w_skip)
         self.w_out = quant(block.w_out)
         self.w_x = torch.cat([block.w_r, block.w_B, block.w_C]).detach().to(dtype)
-        self.w_dt = block.w_dt.detach().to(dtype)
+        self.w_dt = block.w_dt.detach().to(dtype, copy=True)
         self.conv_w, self.conv_b = f32(block.conv_w), f32(block.conv_b)
         self.A = -torch.exp(f32(block.A_log))
         self.D, self.dt_bias = f32(block.D), f32(block.dt_bias)
@@ -53,9 +53,9 @@ class MambaDecoder:
         if not stack.embed.is_cuda:
             raise ValueError("MambaDecoder needs a stack on a CUDA device")
         self.dtype, self.eps = dtype, stack.norm.eps
-        self.embed = stack.embed.detach().float()
+        self.embed = stack.embed.detach().to(torch.float32, copy=True)
         self.layers = [_Layer(b, dtype) for b in stack.layers]
-        self.norm = stack.norm.weight.detach().float().contiguous()
+        self.norm = stack.norm.weight.detach().to(torch.float32, copy=True)
         self.head = quantize_fp8(stack.head.detach().to(dtype))
 
     def _normed(self, branch, h, weight):

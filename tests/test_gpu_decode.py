@@ -151,3 +151,20 @@ def test_refusals():
     with pytest.raises(ValueError, match="uniform"):
         dec.generate(torch.zeros(2, 3, dtype=torch.int64, device="cuda"), 4,
                      uniform=torch.rand(2, 3, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_are_copies(dtype):
+    """A decoder answers the same after its stack has trained on."""
+    from mamba import MambaDecoder
+
+    stack = _stack()
+    dec = MambaDecoder(stack, dtype=dtype)
+    tokens = torch.randint(0, 50, (3, 9), device="cuda")
+    want, state = dec.prefill(tokens)
+    step = dec.step(tokens[:, 0], state)
+    with torch.no_grad():
+        for p in stack.parameters():
+            p.add_(torch.rand_like(p) + 0.5)
+    got, state = dec.prefill(tokens)
+    assert torch.equal(got, want) and torch.equal(dec.step(tokens[:, 0], state), step)
