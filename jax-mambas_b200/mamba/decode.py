@@ -44,6 +44,8 @@ class MambaDecoder:
     The weights are copied at construction. ``prefill`` and ``step`` return
     float32 logits (B, vocab) of the last position; the state they hand on is
     a list of (conv state, scan state) per layer, updated in place by ``step``.
+    The token -1, ``sample_tokens``' answer for a row with nothing to draw, makes
+    that row's logits and state NaN, from which nothing is drawn either: -1 from there on.
     """
 
     def __init__(self, stack, dtype=torch.bfloat16):
@@ -53,7 +55,10 @@ class MambaDecoder:
         if not stack.embed.is_cuda:
             raise ValueError("MambaDecoder needs a stack on a CUDA device")
         self.dtype, self.eps = dtype, stack.norm.eps
-        self.embed = stack.embed.detach().to(torch.float32, copy=True)
+        # one row more, of NaN: what the token -1 indexes
+        self.embed = torch.cat([stack.embed.detach().float(),
+                                stack.embed.new_full((1, stack.embed.shape[1]), float("nan"),
+                                                     dtype=torch.float32)])
         self.layers = [_Layer(b, dtype) for b in stack.layers]
         self.norm = stack.norm.weight.detach().to(torch.float32, copy=True)
         self.head = quantize_fp8(stack.head.detach().to(dtype))

@@ -168,3 +168,30 @@ def test_weights_are_copies(dtype):
             p.add_(torch.rand_like(p) + 0.5)
     got, state = dec.prefill(tokens)
     assert torch.equal(got, want) and torch.equal(dec.step(tokens[:, 0], state), step)
+
+
+def test_rows_with_nothing_to_draw():
+    """-1 is no token of the vocabulary: a row that has it gives NaN, and -1 from there
+    on; the other rows do not notice."""
+    from mamba import MambaDecoder, sample_tokens
+
+    stack = _stack()
+    with torch.no_grad():
+        stack.embed[7] = float("nan")
+    dec = MambaDecoder(stack)
+    tokens = torch.randint(8, 50, (4, 11), device="cuda")
+    u = torch.rand(4, 5, device="cuda")
+    want = dec.generate(tokens, 5, uniform=u)
+    bad = tokens.clone()
+    bad[1, 4] = 7
+    got = dec.generate(bad, 5, uniform=u)
+    assert (got[1] == -1).all() and torch.equal(got[[0, 2, 3]], want[[0, 2, 3]])
+    bad[1, 4], bad[3, 10] = -1, -1
+    logits, state = dec.prefill(bad)
+    plain, plain_state = dec.prefill(tokens)
+    for nxt in (tokens[:, 0], torch.tensor([3, -1, -1, 5], device="cuda"), tokens[:, 2]):
+        gone = logits.isnan().all(1)
+        assert not logits[~gone].isnan().any() and torch.equal(logits[~gone], plain[~gone])
+        assert torch.equal(sample_tokens(logits, u[:, 0]) == -1, gone)
+        logits, plain = dec.step(nxt, state), dec.step(nxt.clamp(min=0), plain_state)
+    assert logits.isnan().all(1).tolist() == [False, True, True, True]
