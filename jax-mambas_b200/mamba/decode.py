@@ -75,11 +75,19 @@ class MambaDecoder:
 
     @torch.no_grad()
     def prefill(self, tokens, seq_lens=None):
-        """tokens (B, L), L >= 1, right-padded to seq_lens (B,) int32 (each >= 1)
-        if given: logits of each row's last token, and the state after it."""
+        """tokens (B, L), L >= 1, right-padded to seq_lens (B,) int32 if given:
+        logits of each row's last token, and the state after it. Lengths above L
+        count as L, as in the conv and the scan; a row of length 0 has NaN logits and
+        the state before any token, from which ``step`` can go on."""
         if tokens.ndim != 2 or tokens.shape[1] < 1:
             raise ValueError("tokens must have shape (B, L) with L >= 1")
         batch, length = tokens.shape
+        if seq_lens is not None:
+            if (seq_lens.shape != (batch,) or seq_lens.dtype != torch.int32
+                    or seq_lens.device != self.embed.device):
+                raise ValueError("seq_lens must be an int32 tensor of shape (B,) on the "
+                                 "weights' device")
+            lens = seq_lens.long().clamp(0, length)
         h = self.embed[tokens].view(batch * length, -1)
         branch, state = None, []
         for p in self.layers:
@@ -88,7 +96,7 @@ class MambaDecoder:
             z = fp8_matmul(q, s, *p.w_skip, out_dtype=self.dtype, channel_major_batch=batch)
             u, conv = causal_conv1d_fn(x, p.conv_w, p.conv_b, seq_lens, return_final_state=True)
             if seq_lens is not None:  # the last inputs of each row, not of the padding
-                at = seq_lens[:, None].long() + torch.arange(1 - p.kw, 0, device=x.device)
+                at = lens[:, None] + torch.arange(1 - p.kw, 0, device=x.device)
                 conv = x.gather(2, at.clamp(min=0)[:, None].expand(-1, p.inner, -1))
                 conv = conv.masked_fill((at < 0)[:, None], 0.0)
             xp = torch.matmul(p.w_x, u)
@@ -101,9 +109,12 @@ class MambaDecoder:
                                 out_dtype=self.dtype)
             state.append((conv, last))
         end = (torch.full((batch,), length, device=tokens.device) if seq_lens is None
-               else seq_lens.long())
+               else lens.clamp(min=1))
         rows = torch.arange(batch, device=tokens.device) * length + end - 1
-        return self._logits(branch[rows], h[rows]), state
+        logits = self._logits(branch[rows], h[rows])
+        if seq_lens is not None:
+            logits.masked_fill_((lens < 1)[:, None], float("nan"))
+        return logits, state
 
     @torch.no_grad()
     def step(self, tokens, state):
@@ -124,7 +135,8 @@ class MambaDecoder:
     @torch.no_grad()
     def generate(self, tokens, new_tokens, seq_lens=None, uniform=None, generator=None,
                  **sampling):
-        """new_tokens further tokens (B, new_tokens) for prompts (B, L).
+        """new_tokens further tokens (B, new_tokens) for prompts (B, L); -1 where
+        a row has nothing to draw.
 
         uniform (B, new_tokens) float32 in [0, 1) fixes the draws; without it
         they come from `generator` (on the tokens' device). sampling:

@@ -195,3 +195,39 @@ def test_rows_with_nothing_to_draw():
         assert torch.equal(sample_tokens(logits, u[:, 0]) == -1, gone)
         logits, plain = dec.step(nxt, state), dec.step(nxt.clamp(min=0), plain_state)
     assert logits.isnan().all(1).tolist() == [False, True, True, True]
+
+
+def test_lengths_outside_the_prompt():
+    """A row of length 0 reads no other row's position: NaN logits and the state before
+    any token; a length above L is L."""
+    from mamba import MambaDecoder
+
+    dec = MambaDecoder(_stack())
+    tokens = torch.randint(0, 50, (5, 30), device="cuda")
+    nxt = torch.randint(0, 50, (5,), device="cuda")
+    logits, state = dec.prefill(
+        tokens, torch.tensor([0, 5, 41, 0, -2], dtype=torch.int32, device="cuda"))
+    assert logits.isnan().all(1).tolist() == [True, False, False, True, True]
+    for conv, scan in state:
+        assert (conv[[0, 3, 4]] == 0).all() and (scan[[0, 3, 4]] == 0).all()
+    want, want_state = dec.prefill(
+        tokens, torch.tensor([1, 5, 30, 7, 2], dtype=torch.int32, device="cuda"))
+    assert torch.equal(logits[1:3], want[1:3])
+    after, want_after = dec.step(nxt, state), dec.step(nxt, want_state)
+    assert torch.equal(after[1:3], want_after[1:3])
+    first = dec.prefill(nxt[:, None])[0]  # the rows' first token
+    assert _rel(after[[0, 3, 4]], first[[0, 3, 4]]) < 0.04
+    got = dec.generate(tokens, 3, seq_lens=torch.tensor([9, 0, 3, 1, 30], dtype=torch.int32,
+                                                        device="cuda"))
+    assert (got[1] == -1).all() and (got[[0, 2, 3, 4]] >= 0).all()
+
+
+def test_lengths_that_are_refused():
+    from mamba import MambaDecoder
+
+    dec = MambaDecoder(_stack())
+    tokens = torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    for bad in (torch.ones(2, dtype=torch.int32), torch.ones(2, device="cuda"),
+                torch.ones(3, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError, match="seq_lens"):
+            dec.prefill(tokens, bad)
