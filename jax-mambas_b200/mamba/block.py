@@ -177,16 +177,17 @@ class MambaStack(nn.Module):
     the reference's induction-heads experiment (configs[3]: 2 layers,
     d_model 64, expand 2, d_state 16, conv 4, RMSNorm, vocab 16).
 
-    fp8_head: the final norm (RMSNorm, the rms_norm_fn kernel, in `dtype`) and
-    the vocabulary projection (fp8_linear: forward and both gradients in 8 bits)
-    run on the kernels; float32 logits."""
+    fp8_head: the final norm (RMSNorm, the rms_norm_fn kernel) and the vocabulary
+    projection (fp8_linear: forward and both gradients in 8 bits) run on the
+    kernels, on the float32 residual stream and weights whatever `dtype`: the
+    only roundings are those to 8 bits, and the logits are the float32 sums."""
 
     def __init__(self, vocab, d_model, n_layers, norm_type="rmsnorm", dtype=torch.float32,
                  device="cuda", seed=0, fp8_head=False, **kw):
         super().__init__()
         if fp8_head and norm_type != "rmsnorm":
             raise ValueError("fp8_head needs norm_type 'rmsnorm'")
-        self.fp8_head, self.head_dtype = fp8_head, dtype
+        self.fp8_head = fp8_head
         g = torch.Generator(device="cpu").manual_seed(seed)
         self.embed = nn.Parameter(torch.randn(vocab, d_model, generator=g) * d_model ** -0.5)
         self.layers = nn.ModuleList(
@@ -202,6 +203,6 @@ class MambaStack(nn.Module):
         for layer in self.layers:
             x = layer(x, seq_lens)
         if self.fp8_head:
-            x = rms_norm_fn(x.to(self.head_dtype), self.norm.weight, eps=self.norm.eps)
-            return fp8_linear(x, self.head.to(self.head_dtype)).float()
+            x = rms_norm_fn(x.float(), self.norm.weight, eps=self.norm.eps)
+            return fp8_linear(x, self.head.float())
         return self.norm(x) @ self.head.t()

@@ -231,3 +231,23 @@ def test_lengths_that_are_refused():
                 torch.ones(3, dtype=torch.int32, device="cuda")):
         with pytest.raises(ValueError, match="seq_lens"):
             dec.prefill(tokens, bad)
+
+
+def test_head_in_8_bits_rounds_to_8_bits_alone():
+    """Norm of the float32 stream, 8-bit operands from its float32 result and the float32
+    weight, float32 sums and gradients: nothing passes through the stack's bfloat16."""
+    from mamba import fp8_matmul, quantize_fp8, rms_norm_fn
+
+    m = _stack(seed=9, fp8_head=True)
+    tokens = torch.randint(0, 50, (4, 33), device="cuda")
+    x = m.embed[tokens]
+    for layer in m.layers:
+        x = layer(x)
+    y = rms_norm_fn(x, m.norm.weight, eps=1e-5).flatten(0, 1).detach()
+    want = fp8_matmul(*quantize_fp8(y), *quantize_fp8(m.head.detach()), out_dtype=torch.float32)
+    out = m(tokens)
+    assert torch.equal(out.flatten(0, 1), want)
+    dy = torch.randn(4 * 33, 50, device="cuda")
+    dhead, = torch.autograd.grad(out, m.head, dy.view(4, 33, 50))
+    assert torch.equal(dhead, fp8_matmul(*quantize_fp8(dy.t()), *quantize_fp8(y.t()),
+                                         out_dtype=torch.float32))
