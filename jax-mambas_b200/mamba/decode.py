@@ -7,7 +7,7 @@ projections are block-scaled 8-bit products (``fp8_matmul``) on weights
 quantised once, prompts run through the conv and scan kernels in their (B, D,
 L) layout, single tokens through the step kernels (Mamba.step,
 mamba/mamba1.py:339-355), and ``sample_tokens`` draws. x_proj and dt_proj stay
-in the stack's bfloat16: they are small, and feed exponentials.
+in the decoder's `dtype`: they are small, and feed exponentials.
 """
 from __future__ import annotations
 
@@ -24,7 +24,7 @@ class _Layer:
     """A MambaBlock's weights as the decoder reads them."""
 
     def __init__(self, block, dtype):
-        quant = lambda w: quantize_fp8(w.detach().to(dtype))  # noqa: E731
+        quant = lambda w: quantize_fp8(w.detach().float())  # noqa: E731
         f32 = lambda w: w.detach().to(torch.float32, copy=True).contiguous()  # noqa: E731
         self.norm = f32(block.norm.weight)
         self.w_main, self.w_skip = quant(block.w_main), quant(block.w_skip)
@@ -61,7 +61,7 @@ class MambaDecoder:
                                                      dtype=torch.float32)])
         self.layers = [_Layer(b, dtype) for b in stack.layers]
         self.norm = stack.norm.weight.detach().to(torch.float32, copy=True)
-        self.head = quantize_fp8(stack.head.detach().to(dtype))
+        self.head = quantize_fp8(stack.head.detach().float())
 
     def _normed(self, branch, h, weight):
         """8-bit norm of the residual stream with the last branch added."""

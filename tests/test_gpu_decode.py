@@ -251,3 +251,17 @@ def test_head_in_8_bits_rounds_to_8_bits_alone():
     dhead, = torch.autograd.grad(out, m.head, dy.view(4, 33, 50))
     assert torch.equal(dhead, fp8_matmul(*quantize_fp8(dy.t()), *quantize_fp8(y.t()),
                                          out_dtype=torch.float32))
+
+
+def test_weights_are_rounded_once():
+    """The 8-bit weights are those of the stack's float32 ones."""
+    from mamba import MambaDecoder, quantize_fp8
+
+    stack = _stack()
+    dec = MambaDecoder(stack)
+    pairs = [(dec.head, stack.head)]
+    for a, b in zip(dec.layers, stack.layers):
+        pairs += [(a.w_main, b.w_main), (a.w_skip, b.w_skip), (a.w_out, b.w_out)]
+    for got, w in pairs:
+        for a, b in zip(got, quantize_fp8(w.detach())):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
