@@ -12,12 +12,14 @@ against its array's extent and report violations through
 ``mamba_ss_take_bounds_violations()`` instead of faulting. Load it in place of
 the normal library with ``MAMBA_SS_B200_LIB``.
 
-``build_torch_extension()`` (part of ``build.py``) builds ``_mamba_ops.so``
-beside it, the host side of the operators around the scan layers for PyTorch.
+``build_torch_extension()`` (part of ``build.py`` where PyTorch is installed) builds
+``_mamba_ops.so`` beside it, the host side of the operators around the scan layers
+for PyTorch. The library itself needs no PyTorch.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -145,6 +147,9 @@ def build_torch_extension(force: bool = False) -> Path:
 
 
 if __name__ == "__main__":
-    build_torch_extension(force="--force" in sys.argv)
     print(build_library(force="--force" in sys.argv, verbose="-v" in sys.argv,
                         bounds="--bounds" in sys.argv))
+    if importlib.util.find_spec("torch") is not None:
+        print(build_torch_extension(force="--force" in sys.argv))
+    else:
+        print(f"PyTorch is not installed: {torch_extension_path().name} not built")

@@ -86,3 +86,19 @@ def test_no_fallback_on_cpu_tensors():
                  lambda: mamba.sample_tokens(x, torch.rand(4))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+@pytest.mark.timeout(900)
+def test_library_builds_without_torch():
+    """The C library serves callers that have no PyTorch; only the operators' PyTorch
+    host side needs it."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    build = Path(__file__).resolve().parents[1] / "jax-mambas_b200" / "build.py"
+    code = ("import runpy, sys; sys.modules['torch'] = None; sys.argv = ['build.py']; "
+            f"runpy.run_path({str(build)!r}, run_name='__main__')")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    assert "libmamba_ss_b200.so" in r.stdout and "_mamba_ops.so not built" in r.stdout
