@@ -102,3 +102,12 @@ def test_library_builds_without_torch():
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
     assert "libmamba_ss_b200.so" in r.stdout and "_mamba_ops.so not built" in r.stdout
+
+
+def test_missing_binding_says_how_to_build_it(lib, monkeypatch, tmp_path):
+    from mamba import _native, _ops
+
+    monkeypatch.setattr(_ops, "_OPS", None)
+    monkeypatch.setattr(_native, "_PKG_ROOT", tmp_path)
+    with pytest.raises(FileNotFoundError, match="build.py"):
+        _ops.ops()
