@@ -148,7 +148,7 @@ mss_status mamba_ss_quantize_fp8(void* stream, int32_t x_dtype, int32_t channel_
   const int64_t kb = (k + 127) / 128;
   if (!grid_ok(length) || batch > (1ll << 40) / length ||
       (channel_major ? batch > 65535 || kb > 65535
-                     : !grid_ok(batch * length * kb)))
+                     : !grid_ok(batch * length) || !grid_ok(batch * length * kb)))
     return bad(op, "sizes too large");
   if (!x || !codes || !scales) return bad(op, "x, codes and scales must be non-null");
   if (!channel_major && x_stride < 0) return bad(op, "row stride must not be negative");

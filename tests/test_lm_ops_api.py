@@ -111,3 +111,10 @@ def test_missing_binding_says_how_to_build_it(lib, monkeypatch, tmp_path):
     monkeypatch.setattr(_native, "_PKG_ROOT", tmp_path)
     with pytest.raises(FileNotFoundError, match="build.py"):
         _ops.ops()
+
+
+def test_row_counts_that_pass_64_bits_are_refused(lib):
+    """2^40 rows of 2^23 blocks are 2^63: no number of 64 bits with a sign."""
+    st = lib.mamba_ss_quantize_fp8(None, 0, 0, 1 << 20, 1 << 20, 1 << 30, P, 1 << 30, P, 1 << 30,
+                                   P, 1 << 23)
+    _says(lib, st, b"too large")
