@@ -491,6 +491,22 @@ struct PairCfg {
   static constexpr int acc(int buf) { return buf == 0 ? kSfCols : 256; }
 };
 
+// What the issuing thread has handed to the tensor cores, as its rings' next places: the
+// arrivals that its commits make on each CTA's barriers.
+struct Issued {
+  uint32_t stages, groups, tiles;  // the rings': place, and phase from bit 8 on
+};
+template <int kN>
+__device__ __forceinline__ uint32_t packed(const Ring<kN>& r) {
+  return static_cast<uint32_t>(r.at) | (r.phase << 8);
+}
+// Waits for the last arrival on each of a ring's barriers (a barrier without one is ready).
+__device__ __forceinline__ void drain_ring(uint64_t* bars, int n, uint32_t next) {
+  const int at = static_cast<int>(next & 0xffu);
+  const uint32_t phase = next >> 8;
+  for (int s = 0; s < n; ++s) mbar_wait_bounded(bars + s, s < at ? phase : phase ^ 1);
+}
+
 // wait_role for barriers that the other CTA arrives at; giving up is told to it.
 __device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, uint32_t polls,
                                           volatile int* gave_up, uint32_t other_flag) {
@@ -499,7 +515,7 @@ __device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, uint32
     if (*gave_up) return false;
   }
   *gave_up = 1;
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(other_flag), "r"(1) : "memory");
+  cluster_st32(other_flag, 1u);
   atomicOr(&g_fp8_err, kErrTmaTimeout);
   return false;
 }
@@ -526,6 +542,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   uint64_t* drained = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile Issued* issued = reinterpret_cast<volatile Issued*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_rank());
@@ -628,6 +645,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       int t = 0, to = 0;
       Ring<kStages> r;
       Ring<kSfSlots> g;
+      Ring<2> done;
       auto copy_scales = [&]() -> bool {  // a group ahead, as above
         if (!wait(sf_full + g.at, g.phase)) return false;
         tc_fence_after();
@@ -668,14 +686,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
           if (byte == kSfGroup - 1 || end) slot ^= 1;
           if (byte == 0 && !(last && b + kSfGroup >= p.kb) && !copy_scales()) {
             ok = false;
+            r.next();
             break;
           }
         }
-        // (after giving up the other CTA may not wait for it any more)
-        if (ok) mma_commit_pair(acc_full + buf);
+        if (ok) {
+          mma_commit_pair(acc_full + buf);
+          done.next();
+        }
       }
       mma_commit_pair_own(drained);
       mbar_wait_bounded(drained, 0);
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t to = cluster_map(smem_u32(const_cast<Issued*>(issued)), q);
+        cluster_st32(to, packed(r));
+        cluster_st32(to + 4, packed(g));
+        cluster_st32(to + 8, packed(done));
+      }
     }
   } else if (warp == 2) {
     const uint32_t to = cluster_map(smem_u32(sf_full), 0);
@@ -705,6 +732,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   }
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves while the other's work reaches into it
+  // After giving up (both know by now) the roles have not waited for the last arrivals of
+  // the products and copies that were issued.
+  if (*gave_up && threadIdx.x == 0) {
+    drain_ring(empty, kStages, issued->stages);
+    drain_ring(sf_empty, kSfSlots, issued->groups);
+    drain_ring(acc_full, 2, issued->tiles);
+  }
   if (warp == 3) tmem_free_pair<Cfg::kTmem>(tmem);
 }
 

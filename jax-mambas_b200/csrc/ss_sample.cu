@@ -130,9 +130,6 @@ __device__ __forceinline__ uint32_t cluster_ld32(uint32_t addr) {
 __device__ __forceinline__ void cluster_st64(uint32_t addr, unsigned long long v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
-__device__ __forceinline__ void cluster_st32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 
 // A shared-memory word of every CTA of the row, zero past the last; the loads are
 // all under way before the first is used.
