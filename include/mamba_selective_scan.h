@@ -51,8 +51,9 @@ const char* mamba_ss_last_error(void);
 const char* mamba_ss_version(void);
 
 /* Returns and clears the device-side error word of the current device:
- * bit 0 = a kernel gave up waiting (bounded) for its TMA copies and returned
- * early, so its outputs are incomplete. Synchronous; no counterpart in the
+ * bit 0 = a kernel gave up waiting (bounded) for its TMA copies, or an 8-bit
+ * product for another of its roles, and returned early, so its outputs are
+ * incomplete. Synchronous; no counterpart in the
  * reference, whose kernels have no waits. */
 uint32_t mamba_ss_take_device_error(void);
 
@@ -93,8 +94,8 @@ void mamba_ss_set_deterministic(int32_t on);
 int32_t mamba_ss_deterministic(void);
 
 /* Test hook for the bounded waits: sets the number of polls after which
- * the scan kernels launched from now on (any host thread) give up waiting
- * for a tile's TMA staging, report bit 0 through
+ * the scan kernels and 8-bit products launched from now on (any host thread)
+ * give up waiting for a tile's TMA staging, report bit 0 through
  * mamba_ss_take_device_error() and return with incomplete outputs (they
  * still let their copies in flight land first). 0 makes every such wait
  * give up at once; a negative value restores the default (2^22 polls, far

@@ -46,7 +46,8 @@ def fp8_matmul(a, a_scale, b, b_scale, out_dtype=torch.bfloat16, channel_major_b
     out_dtype float32 or bfloat16. The result is (M, N); with
     channel_major_batch = B (M = B * L) it is (B, N, L), the scan's layout.
     For inference and as the building block of ``fp8_linear``: 8-bit operands
-    carry no gradient.
+    carry no gradient. A product that gives up a wait leaves its output incomplete
+    and sets bit 0 of the library's device error word (mamba_ss_take_device_error).
     """
     return ops().fp8_matmul(a, a_scale, b, b_scale, out_dtype, channel_major_batch)
 
